@@ -217,7 +217,7 @@ def _prepare_attend(c, seed):
          "recent_lens": torch.tensor(recent_lens, dtype=torch.int32, device=DEV),
          "zones": [_zone(k, v) for k, v in zones]}
     if own:
-        ops = s["ops"] = _library().ops
+        ops = _library().ops
         s["pool"] = ops.Int4Pool(0, h, DEV)
         s["pool"].data, s["pool"].num_blocks = data, total
         s["handles"] = []
@@ -450,7 +450,7 @@ def run(state):
                 "compact": _plain_compact}[kind](state)
     if kind == "attend":
         c = state["case"]
-        return state["ops"].shared_prefix_attention(
+        return _library().ops.shared_prefix_attention(
             state["q"], c["shared"] // BLOCK, group=c["samples"], zones=state["handles"], pool=state["pool"],
             block_table=state["table"], int4_lens=state["lens"], int4_max_len=c["shared"] + c["own"])
     t = state["tables"]
