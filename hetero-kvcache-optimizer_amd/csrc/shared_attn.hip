@@ -137,12 +137,12 @@ __device__ __forceinline__ float row_sum(float v) {
 // Online softmax of NT row tiles.  m is a reference that no score passes by more than nothing: x =
 // s - m <= 0, so 2^x is at most 1.  When a score passes it, m becomes that score + kHeadroom, and
 // the scores a little larger that follow need no new reference and no pass over the
-// accumulators; four bits are taken from the smallest probabilities.  `fresh`: no score yet, m is 0
-// and has to become the first ones' whatever they are.  One branch for all tiles: with a branch
-// for each, no product of one tile could run beside another's exponentials.
+// accumulators; four bits are taken from the smallest probabilities.  `fresh`: a row may have had no
+// score yet, or only -inf, m is 0 and has to go by the first one whatever it is.  One branch for all
+// tiles: with a branch for each, no product of one tile could run beside another's exponentials.
 constexpr float kHeadroom = 4.0f;
 template <int NT, int N>
-__device__ __forceinline__ void raise_reference(bool fresh, float (&x)[NT][N], f4 (&acc)[NT][8], float (&m)[NT], float (&l)[NT]) {
+__device__ __forceinline__ void raise_reference(bool& fresh, float (&x)[NT][N], f4 (&acc)[NT][8], float (&m)[NT], float (&l)[NT]) {
     float top[NT];
     bool any = fresh;
 #pragma unroll
@@ -153,12 +153,15 @@ __device__ __forceinline__ void raise_reference(bool fresh, float (&x)[NT][N], f
         any |= top[nt] > 0.f;
     }
     if (__ballot(any)) {
+        bool waits = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const float t = row_max(top[nt]);
-            const float up = (fresh ? t > -INFINITY : t > 0.f) ? t + kHeadroom : 0.f;
+            const bool first = fresh && row_max(l[nt]) == 0.f;
+            waits |= first && t == -INFINITY;
+            const float up = (first ? t > -INFINITY : t > 0.f) ? t + kHeadroom : 0.f;
             if (__ballot(up != 0.f) == 0) continue;
-            const float a = fresh ? 1.0f : fast_exp2(-up);
+            const float a = first ? 1.0f : fast_exp2(-up);
 #pragma unroll
             for (int i = 0; i < N; ++i) x[nt][i] -= up;
 #pragma unroll
@@ -166,6 +169,7 @@ __device__ __forceinline__ void raise_reference(bool fresh, float (&x)[NT][N], f
             l[nt] *= a;
             m[nt] += up;
         }
+        fresh = fresh && __ballot(waits) != 0;
     }
 }
 // Probabilities relative to the reference, and their sum.
@@ -238,8 +242,8 @@ __device__ __forceinline__ int check_ids(const Params& p, int id) {
 // the queries ready, q(nt, j) is dims 32g + 8j .. +7 of row c of tile nt.
 template <int NT, class Stage, class Q>
 __device__ __forceinline__ void attend_int4(const Params& p, const int32_t* row, int ids, int h, int b0, int b1, int len,
-                                            const Lane& ln, const Stage& stage, const Q& q, f4 (&acc)[NT][8], float (&m)[NT],
-                                            float (&l)[NT]) {
+                                            const Lane& ln, const Stage& stage, const Q& q, bool& fresh, f4 (&acc)[NT][8],
+                                            float (&m)[NT], float (&l)[NT]) {
     Blocks bl;
     if (b0 >= b1) stage();
     for (int wb = b0; wb < b1; wb += kWindow) {
@@ -317,7 +321,7 @@ __device__ __forceinline__ void attend_int4(const Params& p, const int32_t* row,
             load_k(bl.at(iA), ln, kA);
             load_k(bl.at(iB), ln, kB);
             __builtin_amdgcn_sched_barrier(0);
-            raise_reference<NT, 8>(lb == b0, x, acc, m, l);
+            raise_reference<NT, 8>(fresh, x, acc, m, l);
             // ---- V operands and scales
             h8 V0[4], V1[4];
             float vs[8];
@@ -382,9 +386,9 @@ __device__ __forceinline__ void attend_int4(const Params& p, const int32_t* row,
     }
 }
 
-// fp16 tiles [t0, t1), counted over the zones, of sequence b; fresh: as raise_reference's.
+// fp16 tiles [t0, t1), counted over the zones, of sequence b.
 __device__ __forceinline__ void attend_f16(const Params& p, int b, int h, const int (&lens)[HKV_MAX_F16_ZONES], int t0, int t1,
-                                           bool fresh, const Lane& ln, const h8 (&qf)[4], f4 (&acc)[1][8], float (&m)[1],
+                                           const Lane& ln, const h8 (&qf)[4], bool& fresh, f4 (&acc)[1][8], float (&m)[1],
                                            float (&l)[1]) {
     const int64_t bh = (int64_t)b * p.Hkv + h;
     F16Tile buf[2];   // two tiles on their way
@@ -422,7 +426,7 @@ __device__ __forceinline__ void attend_f16(const Params& p, int b, int h, const 
             float x[1][4], pr[4];
 #pragma unroll
             for (int v = 0; v < 4; ++v) x[0][v] = g4 + v < n ? __builtin_fmaf(S[v], p.scale_log2, -m[0]) : -INFINITY;
-            raise_reference<1, 4>(fresh && t + u == t0, x, acc, m, l);
+            raise_reference<1, 4>(fresh, x, acc, m, l);
             exponentiate<4>(x[0], l[0], pr);
             h4 P;
 #pragma unroll
@@ -621,7 +625,8 @@ __device__ __forceinline__ void prefix_range(const Params& p, float* smem, int i
         __syncthreads();
     };
     const auto q = [&](int nt, int j) { return *(const h8*)(sm + ((nt * 4 + j) * 64 + lane) * 16); };
-    attend_int4<NT>(p, row, ids, h, w0, w1, count * kBlockTokens, ln, stage, q, acc, m, l);
+    bool fresh = true;
+    attend_int4<NT>(p, row, ids, h, w0, w1, count * kBlockTokens, ln, stage, q, fresh, acc, m, l);
     float* states = p.states + (int64_t)split * p.B * p.Hkv * p.nrep * kState;
     float* buf = (float*)(sm + query_bytes(NT));
     // two tiles between barriers
@@ -697,13 +702,14 @@ __device__ __forceinline__ void own_range(const Params& p, float* smem, int wg) 
     float m[1] = {0.f}, l[1] = {0.f};
 #pragma unroll
     for (int n = 0; n < 8; ++n) acc[0][n] = f4{0.f, 0.f, 0.f, 0.f};
+    bool fresh = true;
     attend_int4<1>(p, row, ids, h, w0, w1, len, ln, [&]() { query_to_f16(p, qw); },
-                   [&](int, int j) { return __builtin_bit_cast(h8, qw[j]); }, acc, m, l);
+                   [&](int, int j) { return __builtin_bit_cast(h8, qw[j]); }, fresh, acc, m, l);
     if (f1 > f0) {
         h8 qf[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) qf[j] = __builtin_bit_cast(h8, qw[j]);
-        attend_f16(p, b, h, lens, f0, f1, w1 <= w0, ln, qf, acc, m, l);
+        attend_f16(p, b, h, lens, f0, f1, ln, qf, fresh, acc, m, l);
     }
     float* states = p.states + ((int64_t)(p.prefix_ranges + split) * p.B + b) * Hq * kState + (int64_t)h * p.nrep * kState;
     if (p.own_waves == 1) {
