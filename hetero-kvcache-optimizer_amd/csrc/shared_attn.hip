@@ -134,15 +134,24 @@ __device__ __forceinline__ float row_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Online softmax of NT row tiles.  m is a reference that no score passes by more than nothing: x =
-// s - m <= 0, so 2^x is at most 1.  When a score passes it, m becomes that score + kHeadroom, and
-// the scores a little larger that follow need no new reference and no pass over the
-// accumulators; four bits are taken from the smallest probabilities.  `fresh`: a row may have had no
-// score yet, or only -inf, m is 0 and has to go by the first one whatever it is.  One branch for all
-// tiles: with a branch for each, no product of one tile could run beside another's exponentials.
+// Online softmax of NT row tiles.  m is a reference, and the scores relative to it, x = s - m, are at
+// most `lim`.  What limits them is fp16: P = 2^x times a token's V scale goes into the products as
+// fp16, so lim + log2 of the largest V scale (or a little more) is kTopP.  Thus P uses fp16's upper end
+// whatever the size of V, and the likeliest token of V scales within a factor of 4 has 22 bits above the
+// subnormals (with P <= V scale, V of some 2^-8 would have 5).  When a score passes lim, m rises
+// until it is kHeadroom below, and the scores a little larger that follow need no new reference and no
+// pass over the accumulators.  `fresh`: a row may have had no score yet, or only -inf, and its m has to
+// go by the first one whatever it is.  One branch for all tiles: with a branch for each, no product
+// of one tile could run beside another's exponentials.
 constexpr float kHeadroom = 4.0f;
+constexpr int kTopP = 15;
+struct Range {
+    float lim = kTopP;
+    float largest = 0.f;   // V scale that lim allows
+};
 template <int NT, int N>
-__device__ __forceinline__ void raise_reference(bool& fresh, float (&x)[NT][N], f4 (&acc)[NT][8], float (&m)[NT], float (&l)[NT]) {
+__device__ __forceinline__ void raise_reference(bool& fresh, float lim, float (&x)[NT][N], f4 (&acc)[NT][8], float (&m)[NT],
+                                                float (&l)[NT]) {
     float top[NT];
     bool any = fresh;
 #pragma unroll
@@ -150,7 +159,7 @@ __device__ __forceinline__ void raise_reference(bool& fresh, float (&x)[NT][N], 
         top[nt] = x[nt][0];
 #pragma unroll
         for (int i = 1; i < N; ++i) top[nt] = fmaxf(top[nt], x[nt][i]);
-        any |= top[nt] > 0.f;
+        any |= top[nt] > lim;
     }
     if (__ballot(any)) {
         bool waits = false;
@@ -159,7 +168,7 @@ __device__ __forceinline__ void raise_reference(bool& fresh, float (&x)[NT][N], 
             const float t = row_max(top[nt]);
             const bool first = fresh && row_max(l[nt]) == 0.f;
             waits |= first && t == -INFINITY;
-            const float up = (first ? t > -INFINITY : t > 0.f) ? t + kHeadroom : 0.f;
+            const float up = (first ? t > -INFINITY : t > lim) ? t - (lim - kHeadroom) : 0.f;
             if (__ballot(up != 0.f) == 0) continue;
             const float a = first ? 1.0f : fast_exp2(-up);
 #pragma unroll
@@ -171,6 +180,33 @@ __device__ __forceinline__ void raise_reference(bool& fresh, float (&x)[NT][N], 
         }
         fresh = fresh && __ballot(waits) != 0;
     }
+}
+// Another limit (uniform), and the references for it.
+template <int NT>
+__device__ __forceinline__ float set_limit(Range& range, float lim, f4 (&acc)[NT][8], float (&m)[NT], float (&l)[NT]) {
+    const float up = range.lim - lim, a = fast_exp2(-up);
+    range.lim = lim;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int n = 0; n < 8; ++n) acc[nt][n] *= a;
+        l[nt] *= a;
+        m[nt] += up;
+    }
+    return up;
+}
+// The limit for V scales up to `top` (a lane's), and up to twice as large ones, which seldom call for
+// another.  Scales of 0 to 2^-47 are alike, and beyond 2^53 P may leave fp16.
+template <int NT, int N>
+__device__ __forceinline__ void fit_scales(Range& range, float top, float (&x)[NT][N], f4 (&acc)[NT][8], float (&m)[NT],
+                                           float (&l)[NT]) {
+    const int e = min(max((int)(__builtin_amdgcn_readfirstlane(__float_as_uint(row_max(top))) >> 23) - 127, -47), 53) + 2;
+    range.largest = __uint_as_float((uint32_t)(e + 127) << 23);
+    const float up = set_limit<NT>(range, (float)(kTopP - e), acc, m, l);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[nt][i] -= up;
 }
 // Probabilities relative to the reference, and their sum.
 template <int N>
@@ -242,8 +278,8 @@ __device__ __forceinline__ int check_ids(const Params& p, int id) {
 // the queries ready, q(nt, j) is dims 32g + 8j .. +7 of row c of tile nt.
 template <int NT, class Stage, class Q>
 __device__ __forceinline__ void attend_int4(const Params& p, const int32_t* row, int ids, int h, int b0, int b1, int len,
-                                            const Lane& ln, const Stage& stage, const Q& q, bool& fresh, f4 (&acc)[NT][8],
-                                            float (&m)[NT], float (&l)[NT]) {
+                                            const Lane& ln, const Stage& stage, const Q& q, bool& fresh, Range& range,
+                                            f4 (&acc)[NT][8], float (&m)[NT], float (&l)[NT]) {
     Blocks bl;
     if (b0 >= b1) stage();
     for (int wb = b0; wb < b1; wb += kWindow) {
@@ -321,10 +357,27 @@ __device__ __forceinline__ void attend_int4(const Params& p, const int32_t* row,
             load_k(bl.at(iA), ln, kA);
             load_k(bl.at(iB), ln, kB);
             __builtin_amdgcn_sched_barrier(0);
-            raise_reference<NT, 8>(fresh, x, acc, m, l);
-            // ---- V operands and scales
-            h8 V0[4], V1[4];
+            raise_reference<NT, 8>(fresh, range.lim, x, acc, m, l);
+            // ---- V scales and operands
             float vs[8];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                vs[v] = vA.s[v];
+                vs[4 + v] = vB.s[v];
+            }
+            if (!full) {
+                asm volatile("");
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    vs[v] = 4 * ln.g + v < nA ? vs[v] : 0.f;
+                    vs[4 + v] = 4 * ln.g + v < nB ? vs[4 + v] : 0.f;
+                }
+            }
+            float scale = 0.f;
+#pragma unroll
+            for (int v = 0; v < 8; ++v) scale = fmaxf(scale, fabsf(vs[v]));
+            if (__ballot(scale > range.largest)) fit_scales<NT, 8>(range, scale, x, acc, m, l);
+            h8 V0[4], V1[4];
             {
                 const h2 zA01 = zp1024(vA.z & 0xffu, (vA.z >> 8) & 0xffu), zA23 = zp64((vA.z >> 16) & 0xffu, vA.z >> 24);
                 const h2 zB01 = zp1024(vB.z & 0xffu, (vB.z >> 8) & 0xffu), zB23 = zp64((vB.z >> 16) & 0xffu, vB.z >> 24);
@@ -333,19 +386,6 @@ __device__ __forceinline__ void attend_int4(const Params& p, const int32_t* row,
                     const NibPairs a = unpack_word(vA.w[mm], zA01, zA23), b = unpack_word(vB.w[mm], zB01, zB23);
                     V0[mm] = h8{a.p0[0], a.p0[1], a.p1[0], a.p1[1], b.p0[0], b.p0[1], b.p1[0], b.p1[1]};
                     V1[mm] = h8{a.p2[0], a.p2[1], a.p3[0], a.p3[1], b.p2[0], b.p2[1], b.p3[0], b.p3[1]};
-                }
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    vs[v] = vA.s[v];
-                    vs[4 + v] = vB.s[v];
-                }
-                if (!full) {
-                    asm volatile("");
-#pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        vs[v] = 4 * ln.g + v < nA ? vs[v] : 0.f;
-                        vs[4 + v] = 4 * ln.g + v < nB ? vs[4 + v] : 0.f;
-                    }
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -386,10 +426,11 @@ __device__ __forceinline__ void attend_int4(const Params& p, const int32_t* row,
     }
 }
 
-// fp16 tiles [t0, t1), counted over the zones, of sequence b.
+// fp16 tiles [t0, t1), counted over the zones, of sequence b.  There is no V scale in their P.
 __device__ __forceinline__ void attend_f16(const Params& p, int b, int h, const int (&lens)[HKV_MAX_F16_ZONES], int t0, int t1,
-                                           const Lane& ln, const h8 (&qf)[4], bool& fresh, f4 (&acc)[1][8], float (&m)[1],
-                                           float (&l)[1]) {
+                                           const Lane& ln, const h8 (&qf)[4], bool& fresh, Range& range, f4 (&acc)[1][8],
+                                           float (&m)[1], float (&l)[1]) {
+    if (range.lim != kTopP) set_limit<1>(range, kTopP, acc, m, l);
     const int64_t bh = (int64_t)b * p.Hkv + h;
     F16Tile buf[2];   // two tiles on their way
     int valid[2];
@@ -426,7 +467,7 @@ __device__ __forceinline__ void attend_f16(const Params& p, int b, int h, const 
             float x[1][4], pr[4];
 #pragma unroll
             for (int v = 0; v < 4; ++v) x[0][v] = g4 + v < n ? __builtin_fmaf(S[v], p.scale_log2, -m[0]) : -INFINITY;
-            raise_reference<1, 4>(fresh, x, acc, m, l);
+            raise_reference<1, 4>(fresh, kTopP, x, acc, m, l);
             exponentiate<4>(x[0], l[0], pr);
             h4 P;
 #pragma unroll
@@ -626,7 +667,8 @@ __device__ __forceinline__ void prefix_range(const Params& p, float* smem, int i
     };
     const auto q = [&](int nt, int j) { return *(const h8*)(sm + ((nt * 4 + j) * 64 + lane) * 16); };
     bool fresh = true;
-    attend_int4<NT>(p, row, ids, h, w0, w1, count * kBlockTokens, ln, stage, q, fresh, acc, m, l);
+    Range range;
+    attend_int4<NT>(p, row, ids, h, w0, w1, count * kBlockTokens, ln, stage, q, fresh, range, acc, m, l);
     float* states = p.states + (int64_t)split * p.B * p.Hkv * p.nrep * kState;
     float* buf = (float*)(sm + query_bytes(NT));
     // two tiles between barriers
@@ -703,13 +745,14 @@ __device__ __forceinline__ void own_range(const Params& p, float* smem, int wg) 
 #pragma unroll
     for (int n = 0; n < 8; ++n) acc[0][n] = f4{0.f, 0.f, 0.f, 0.f};
     bool fresh = true;
+    Range range;
     attend_int4<1>(p, row, ids, h, w0, w1, len, ln, [&]() { query_to_f16(p, qw); },
-                   [&](int, int j) { return __builtin_bit_cast(h8, qw[j]); }, fresh, acc, m, l);
+                   [&](int, int j) { return __builtin_bit_cast(h8, qw[j]); }, fresh, range, acc, m, l);
     if (f1 > f0) {
         h8 qf[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) qf[j] = __builtin_bit_cast(h8, qw[j]);
-        attend_f16(p, b, h, lens, f0, f1, ln, qf, fresh, acc, m, l);
+        attend_f16(p, b, h, lens, f0, f1, ln, qf, fresh, range, acc, m, l);
     }
     float* states = p.states + ((int64_t)(p.prefix_ranges + split) * p.B + b) * Hq * kState + (int64_t)h * p.nrep * kState;
     if (p.own_waves == 1) {
