@@ -850,7 +850,7 @@ __global__ __launch_bounds__(kCombine * 64) void shared_combine_kernel(Params p)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(e), min(i + j, 63)));   // past k: 0
-                const bool in = i + j >= first;
+                const bool in = i + j >= first && i + j < k;   // (past k: state k - 1 may have no part either)
                 o0 = __builtin_fmaf(in ? o[j].x : 0.f, w, o0);
                 o1 = __builtin_fmaf(in ? o[j].y : 0.f, w, o1);
                 if (i + 8 < k) o[j] = *(const f2*)(st + min(i + 8 + j, k - 1) * kWavesRow * stride + 2 * lane);

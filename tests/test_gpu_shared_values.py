@@ -114,3 +114,13 @@ def test_scores_of_minus_infinity_before_small_ones():
     c.keys = [[k[b][:, ~out].double()] for b in range(40)]
     c.values = [[v[b][:, ~out].double()] for b in range(40)]
     c.check(int4_max_len=0, pool=None, block_table=None, int4_lens=None)
+
+
+@pytest.mark.parametrize("shared", [512, 1024, 1600, 2048, 3328, 4000, 6000, 9600])
+def test_what_the_workspace_held_before_does_not_matter(shared):
+    """Of sequences that do not hold the prefix, its states are not written: NaN stays there."""
+    c = Case(52, 1, 3, 32, 8, shared, [20, 3, 0])
+    ws = torch.full((32 << 20,), 255, dtype=torch.uint8, device=DEV)
+    for keep in ([7, shared - 1, 16], [shared + 20, 5, 0], [0, 0, 1], [1, shared + 3, shared]):
+        ws.fill_(255)
+        c.check(keep=keep, int4_lens=torch.tensor(keep, dtype=torch.int32, device=DEV), workspace=ws)
