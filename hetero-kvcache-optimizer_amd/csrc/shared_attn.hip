@@ -13,7 +13,9 @@
 // work and the nibble decode, whose times mostly add to the products'.
 //
 // Work.  One launch: workgroups for ranges of the prefix and for the sequences' own tokens, every
-// range leaving its state (o[128], m, l) in the workspace.  Few states are merged by whoever
+// range leaving its state (o[128], m, l) in the workspace.  A sequence need not hold all of the prefix
+// (its length or its group's count is short of it): its own blocks in there, "strays", are
+// attended by the workgroups of the prefix, all of them, behind what they do for the group.  Few states are merged by whoever
 // stores the last one of a (sequence, kv head) (kJoin), many by a second launch.  A wave
 // streams its own run of block pairs, decodes a pair once into MFMA operands and multiplies it
 // with NT tiles of 16 query rows, NT = 1 .. 4: the decode (~150 of ~400 VALU instructions at NT =
@@ -78,12 +80,13 @@ struct Params {
     uint16_t* out;
     int64_t o_sb, o_sh;
     int* err;
-    float* states;              // [prefix ranges + own ranges][B * Hq][kState]
+    float* states;              // [prefix ranges + own ranges + strays][B * Hq][kState]
     int* arrivals;              // [B][Hkv], with kJoin: states stored, zero again at the end
     const int32_t* counts;      // shared blocks of each group (null: shared_blocks)
     int shared_blocks;
     int row_tiles;              // workgroups of rows per prefix range
     int prefix_ranges, own_ranges;
+    int strays;                 // states of a sequence's strays: as many as prefix ranges, or there can be none
     int own_waves;              // waves per own range: 1, or a workgroup's
     int prefix_wgs, own_wgs;
     int own_first;              // the order of these two kinds of workgroups: the longer ones first
@@ -92,11 +95,20 @@ struct Params {
 __device__ __forceinline__ int row_len(const Params& p, int b) {
     return p.int4_lens ? min(max(load_uniform_i32(p.int4_lens, b), 0), p.int4_max_len) : p.int4_max_len;
 }
-// Shared blocks of a group.  A sequence shorter than these attends all of its tokens as its own.
+// Shared blocks of a group.  A sequence shorter than these has no part in them.
 __device__ __forceinline__ int shared_count(const Params& p, int group) {
     const int n = p.counts ? min(max(load_uniform_i32(p.counts, group), 0), p.shared_blocks) : p.shared_blocks;
     return min(n, p.int4_max_len / kBlockTokens);
 }
+
+// What a sequence of `len` tokens has of the first shared_blocks blocks beside its group's `count`
+// shared ones: blocks [from, to).
+struct Strays {
+    int from, to;
+    __device__ __forceinline__ Strays(const Params& p, int len, int count)
+        : from(len >= count * kBlockTokens ? count : 0), to(min((len + kBlockTokens - 1) / kBlockTokens, p.shared_blocks)) {}
+    __device__ __forceinline__ bool any() const { return from < to; }
+};
 
 // Row c's query values as an MFMA operand takes them: dims 32g + 8j .. +7 (at: dim 32g), zeros
 // without a row.
@@ -543,17 +555,28 @@ __device__ __forceinline__ void merge_get(const float* sm, float* states, const 
 // ---- the merge without a second launch
 // The sums of shared_combine_kernel<1>, in its order, for pieces of rows: a thread merges dims d ..
 // d + 3 of kRows rows (row[i] < 0: none; seq[i]: its sequence; states before first[i] have no part
-// in it), whose states' loads are all on their way at once.
+// in it, those of its strays if stray[i]), whose states' loads are all on their way at once.
+struct Sums {
+    float m, l;
+    f4 o;
+};
+__device__ __forceinline__ Sums add_sums(const Sums& a, const Sums& b) {
+    const float m = fmaxf(a.m, b.m), wa = a.m == -INFINITY ? 0.f : fast_exp2(a.m - m), wb = b.m == -INFINITY ? 0.f : fast_exp2(b.m - m);
+    Sums r = {m, __builtin_fmaf(b.l, wb, a.l * wa), {}};
+#pragma unroll
+    for (int v = 0; v < 4; ++v) r.o[v] = __builtin_fmaf(b.o[v], wb, a.o[v] * wa);
+    return r;
+}
 template <int kRows>
-__device__ __forceinline__ void join_rows(const Params& p, const int (&row)[kRows], const int (&seq)[kRows],
-                                          const int (&first)[kRows], int d) {
-    const int Hq = p.Hkv * p.nrep, T = p.prefix_ranges + p.own_ranges;
+__device__ __forceinline__ void join_states(const Params& p, int from, int n, const int (&row)[kRows], const int (&first)[kRows],
+                                            int d, Sums (&sums)[kRows]) {
+    const int Hq = p.Hkv * p.nrep;
     f4 o[kRows][kJoinFew];
     f2 ml[kRows][kJoinFew];
 #pragma unroll
     for (int k = 0; k < kJoinFew; ++k)
-        if (k < T) {
-            const auto r = rsrc(p.states + (int64_t)k * p.B * Hq * kState, -1);
+        if (k < n) {
+            const auto r = rsrc(p.states + (int64_t)(from + k) * p.B * Hq * kState, -1);
 #pragma unroll
             for (int i = 0; i < kRows; ++i) {
                 const uint32_t at = (uint32_t)max(row[i], 0) * (kState * 4u);
@@ -563,15 +586,14 @@ __device__ __forceinline__ void join_rows(const Params& p, const int (&row)[kRow
         }
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-        if (row[i] < 0) continue;
         float M = -INFINITY, e[8] = {};
         f4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < kJoinFew; ++k)
-            if (k < T && k >= first[i]) M = fmaxf(M, ml[i][k].x);
+            if (k < n && k >= first[i]) M = fmaxf(M, ml[i][k].x);
 #pragma unroll
         for (int k = 0; k < kJoinFew; ++k)
-            if (k < T && k >= first[i]) {
+            if (k < n && k >= first[i]) {
                 const float w = ml[i][k].x == -INFINITY ? 0.f : fast_exp2(ml[i][k].x - M);
                 e[k] = ml[i][k].y * w;
 #pragma unroll
@@ -581,10 +603,30 @@ __device__ __forceinline__ void join_rows(const Params& p, const int (&row)[kRow
         for (int x = 1; x < 8; x <<= 1)
 #pragma unroll
             for (int k = 0; k < 8; k += 2 * x) e[k] += e[k + x];
-        const float inv = e[0] > 0.f ? 1.0f / e[0] : e[0];
+        sums[i] = {M, e[0], O};
+    }
+}
+template <int kRows>
+__device__ __forceinline__ void join_rows(const Params& p, const int (&row)[kRows], const int (&seq)[kRows],
+                                          const int (&first)[kRows], const bool (&stray)[kRows], int d) {
+    const int Hq = p.Hkv * p.nrep, T = p.prefix_ranges + p.own_ranges;
+    Sums sums[kRows];
+    join_states<kRows>(p, 0, T, row, first, d, sums);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        if (row[i] < 0) continue;
+        if (__builtin_expect(stray[i], 0)) {
+            const int one[1] = {row[i]}, all[1] = {0};
+            Sums more[1];
+            int from = T, n = p.strays;
+            asm volatile("" : "+s"(from), "+s"(n));   // (its addresses are for this branch alone)
+            join_states<1>(p, from, n, one, all, d, more);
+            sums[i] = add_sums(sums[i], more[0]);
+        }
+        const float inv = sums[i].l > 0.f ? 1.0f / sums[i].l : sums[i].l;
         uint16_t* to = p.out + (int64_t)seq[i] * p.o_sb + (int64_t)(row[i] - seq[i] * Hq) * p.o_sh + d;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) to[v] = p.out_bf16 ? f2bf_rn(O[v] * inv) : f2h_rn(O[v] * inv);
+        for (int v = 0; v < 4; ++v) to[v] = p.out_bf16 ? f2bf_rn(sums[i].o[v] * inv) : f2h_rn(sums[i].o[v] * inv);
     }
 }
 // One more state of (b, h) is stored, by a range of the prefix (work or none) or of own tokens;
@@ -606,47 +648,11 @@ __device__ __forceinline__ void states_stored() {
 // The queries of a workgroup's row tiles in LDS: [tile][j][lane] operands of 16 bytes.
 constexpr int query_bytes(int tiles) { return tiles * 4096; }
 
+// Blocks [w0, w1) (a wave's) of a group's `count` shared ones, which table row `row` names, against rows
+// r0 .. of the group.
 template <int NT, bool kJoin>
-__device__ __forceinline__ void prefix_range(const Params& p, float* smem, int id) {
-    const int pairs = p.B / p.group * p.Hkv;
-    // workgroups of the row tiles of one range follow one another on one XCD
-    const int rest = id / kXcc, rt = rest % p.row_tiles;
-    const int u = rest / p.row_tiles * kXcc + id % kXcc;
-    if (u >= pairs * p.prefix_ranges) return;
-    const int split = u / pairs, pair = u - split * pairs, group = pair / p.Hkv, h = pair - group * p.Hkv;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Lane ln{lane & 15, lane >> 4, 8 * (lane & 3)};
-    const int count = shared_count(p, group), b0 = group * p.group;
-    if (count <= 0) return;
-    // the range's block pairs, in runs of the waves
-    const int np = (count + 1) >> 1, q0 = np * split / p.prefix_ranges, q1 = np * (split + 1) / p.prefix_ranges;
-    const int w0 = 2 * (q0 + (q1 - q0) * wave / kWaves), w1 = min(2 * (q0 + (q1 - q0) * (wave + 1) / kWaves), count);
-    // the first sequence that holds the shared blocks names them: nearly always the group's
-    // first, whose ids are asked for before the lengths are known
-    const int32_t* row = p.bt + (int64_t)b0 * p.bt_stride;
-    const int n0 = min(kWindow, w1 - w0);
-    int ids = n0 > 0 ? request_ids(row, w0, n0) : 0;
-    const int R = p.group * p.nrep, r0 = rt * NT * 16;
-    u4 qw[4];
-    {   // wave nt of the first NT: row tile nt's queries
-        const int r = r0 + wave * 16 + ln.c;
-        const bool has = wave < NT && r < R;
-        const int b = b0 + (has ? r / p.nrep : 0), hd = h * p.nrep + (has ? r % p.nrep : 0);
-        load_query(p.q + (int64_t)b * p.q_sb + (int64_t)hd * p.q_sh + 32 * ln.g, has, qw);
-    }
-    if (p.int4_lens) {
-        int lead = -1;
-        for (int i = 0; i < p.group && lead < 0; i += 64) {
-            const uint64_t has = __ballot(i + lane < p.group && p.int4_lens[b0 + min(i + lane, p.group - 1)] >= count * kBlockTokens);
-            if (has) lead = i + __builtin_ctzll(has);
-        }
-        if (lead < 0) return;   // nobody holds them: the merge leaves these states out
-        if (lead > 0) {
-            row += (int64_t)lead * p.bt_stride;
-            ids = n0 > 0 ? request_ids(row, w0, n0) : 0;
-        }
-    }
-
+__device__ __forceinline__ void prefix_rows(const Params& p, float* smem, int split, int b0, int h, int r0, const int32_t* row,
+                                            int ids, int w0, int w1, int count, u4 (&qw)[4]) {
     f4 acc[NT][8];
     float m[NT], l[NT];
 #pragma unroll
@@ -657,6 +663,8 @@ __device__ __forceinline__ void prefix_range(const Params& p, float* smem, int i
         for (int n = 0; n < 8; ++n) acc[nt][n] = f4{0.f, 0.f, 0.f, 0.f};
     }
     uint8_t* sm = (uint8_t*)smem;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), R = p.group * p.nrep;
+    const Lane ln{lane & 15, lane >> 4, 8 * (lane & 3)};
     const auto stage = [&]() {
         if (wave < NT) {
             query_to_f16(p, qw);
@@ -687,6 +695,91 @@ __device__ __forceinline__ void prefix_range(const Params& p, float* smem, int i
     }
 }
 
+// A wave's blocks [w0, w1) of a sequence, which table row `row` names, against its rows.
+__device__ __forceinline__ void own_rows(const Params& p, int h, const int32_t* row, int ids, int w0, int w1, int len,
+                                         const Lane& ln, u4 (&qw)[4], bool& fresh, Range& range, f4 (&acc)[1][8], float (&m)[1],
+                                         float (&l)[1]) {
+#pragma unroll
+    for (int n = 0; n < 8; ++n) acc[0][n] = f4{0.f, 0.f, 0.f, 0.f};
+    attend_int4<1>(p, row, ids, h, w0, w1, len, ln, [&]() { query_to_f16(p, qw); },
+                   [&](int, int j) { return __builtin_bit_cast(h8, qw[j]); }, fresh, range, acc, m, l);
+}
+
+// A range's part of the strays of sequences s0 + i, bit i of `which` (buf: behind the last merge).
+template <bool kJoin>
+__device__ __forceinline__ void stray_ranges(const Params& p, float* buf, int split, int h, int s0, int count, uint64_t which) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Lane ln{lane & 15, lane >> 4, 8 * (lane & 3)};
+    const int Hq = p.Hkv * p.nrep;
+    for (; which != 0; which &= which - 1) {
+        const int b = s0 + __builtin_ctzll(which), len = row_len(p, b);
+        const Strays st(p, len, count);
+        const int nb = st.to - st.from, np = (nb + 1) >> 1, parts = p.prefix_ranges * kWaves, part = split * kWaves + wave;
+        const int w0 = st.from + 2 * (np * part / parts), w1 = st.from + min(2 * (np * (part + 1) / parts), nb);
+        const int32_t* row = p.bt + (int64_t)b * p.bt_stride;
+        const int ids = w1 > w0 ? request_ids(row, w0, min(kWindow, w1 - w0)) : 0;
+        u4 qw[4];
+        const bool has = ln.c < p.nrep;
+        load_query(p.q + (int64_t)b * p.q_sb + (int64_t)(h * p.nrep + (has ? ln.c : 0)) * p.q_sh + 32 * ln.g, has, qw);
+        f4 acc[1][8];
+        float m[1] = {0.f}, l[1] = {0.f};
+        bool fresh = true;
+        Range range;
+        own_rows(p, h, row, ids, w0, w1, len, ln, qw, fresh, range, acc, m, l);
+        __syncthreads();   // the merge before this one has been read
+        merge_put(buf, wave, ln, acc[0], m[0], l[0]);
+        __syncthreads();
+        float* states = p.states + ((int64_t)(p.prefix_ranges + p.own_ranges + split) * p.B + b) * Hq * kState + (int64_t)h * p.nrep * kState;
+        merge_get<kJoin>(buf, states, [&](int i) { return i < p.nrep ? i : -1; });
+    }
+}
+
+template <int NT, bool kJoin>
+__device__ __forceinline__ void prefix_range(const Params& p, float* smem, int id) {
+    const int pairs = p.B / p.group * p.Hkv;
+    // workgroups of the row tiles of one range follow one another on one XCD
+    const int rest = id / kXcc, rt = rest % p.row_tiles;
+    const int u = rest / p.row_tiles * kXcc + id % kXcc;
+    if (u >= pairs * p.prefix_ranges) return;
+    const int split = u / pairs, pair = u - split * pairs, group = pair / p.Hkv, h = pair - group * p.Hkv;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Lane ln{lane & 15, lane >> 4, 8 * (lane & 3)};
+    const int count = shared_count(p, group), b0 = group * p.group;
+    // the range's block pairs, in runs of the waves
+    const int np = (count + 1) >> 1, q0 = np * split / p.prefix_ranges, q1 = np * (split + 1) / p.prefix_ranges;
+    const int w0 = 2 * (q0 + (q1 - q0) * wave / kWaves), w1 = min(2 * (q0 + (q1 - q0) * (wave + 1) / kWaves), count);
+    // the first sequence that holds the shared blocks names them: nearly always the group's
+    // first, whose ids are asked for before the lengths are known
+    const int32_t* row = p.bt + (int64_t)b0 * p.bt_stride;
+    const int n0 = min(kWindow, w1 - w0);
+    int ids = n0 > 0 ? request_ids(row, w0, n0) : 0;
+    const int R = p.group * p.nrep, r0 = rt * NT * 16;
+    // lane i: the i-th of the sequences (64 at most) whose first rows are in these tiles
+    const int s0 = b0 + (r0 + p.nrep - 1) / p.nrep, ns = min(b0 + p.group, b0 + (r0 + NT * 16 + p.nrep - 1) / p.nrep) - s0;
+    u4 qw[4];
+    {   // wave nt of the first NT: row tile nt's queries
+        const int r = r0 + wave * 16 + ln.c;
+        const bool has = wave < NT && r < R;
+        const int b = b0 + (has ? r / p.nrep : 0), hd = h * p.nrep + (has ? r % p.nrep : 0);
+        load_query(p.q + (int64_t)b * p.q_sb + (int64_t)hd * p.q_sh + 32 * ln.g, has, qw);
+    }
+    int lead = count > 0 ? 0 : -1, len = p.int4_max_len;   // (lead -1: nobody holds the shared blocks)
+    if (p.int4_lens) {
+        len = min(p.int4_lens[min(s0 + lane, p.B - 1)], p.int4_max_len);
+        lead = -1;
+        for (int i = 0; i < p.group && lead < 0 && count > 0; i += 64) {
+            const uint64_t has = __ballot(i + lane < p.group && p.int4_lens[b0 + min(i + lane, p.group - 1)] >= count * kBlockTokens);
+            if (has) lead = i + __builtin_ctzll(has);
+        }
+        if (lead > 0) {
+            row += (int64_t)lead * p.bt_stride;
+            ids = n0 > 0 ? request_ids(row, w0, n0) : 0;
+        }
+    }
+    const uint64_t strays = __ballot(p.strays > 0 && lane < ns && Strays(p, len, count).any());
+    if (lead >= 0) prefix_rows<NT, kJoin>(p, smem, split, b0, h, r0, row, ids, w0, w1, count, qw);
+    if (__builtin_expect(strays != 0, 0)) stray_ranges<kJoin>(p, smem + query_bytes(NT) / sizeof(float), split, h, s0, count, strays);
+}
 // Behind prefix_range of a group's only row tile: the merge of the sequences whose last state
 // this workgroup stored.
 __device__ __forceinline__ void prefix_join(const Params& p, float* smem, int id) {
@@ -697,6 +790,7 @@ __device__ __forceinline__ void prefix_join(const Params& p, float* smem, int id
     const int b = b0 + min(s, p.group - 1), count = shared_count(p, group);
     const int len = p.int4_lens ? min(p.int4_lens[b], p.int4_max_len) : p.int4_max_len;
     const int first[1] = {count > 0 && len >= count * kBlockTokens ? 0 : p.prefix_ranges}, seq[1] = {b};
+    const bool stray[1] = {p.strays > 0 && Strays(p, len, count).any()};
     states_stored();
     __syncthreads();
     int* last = (int*)smem;
@@ -709,7 +803,7 @@ __device__ __forceinline__ void prefix_join(const Params& p, float* smem, int id
     const int mask = *last;
     if (mask == 0) return;
     const int row[1] = {s < p.group && (mask >> s & 1) ? b * (p.Hkv * p.nrep) + h * p.nrep + i - s * p.nrep : -1};
-    join_rows<1>(p, row, seq, first, d);
+    join_rows<1>(p, row, seq, first, stray, d);
 }
 
 template <bool kJoin>
@@ -723,8 +817,7 @@ __device__ __forceinline__ void own_range(const Params& p, float* smem, int wg) 
     u4 qw[4];
     const bool has = ln.c < p.nrep;
     load_query(p.q + (int64_t)b * p.q_sb + (int64_t)(h * p.nrep + (has ? ln.c : 0)) * p.q_sh + 32 * ln.g, has, qw);
-    const int len = row_len(p, b), count = p.shared_blocks > 0 ? shared_count(p, b / p.group) : 0;
-    const int s0 = len >= count * kBlockTokens ? count : 0;
+    const int len = row_len(p, b), all = (len + kBlockTokens - 1) / kBlockTokens, s0 = min(p.shared_blocks, all);
     int lens[HKV_MAX_F16_ZONES], tiles = 0;
 #pragma unroll
     for (int i = 0; i < HKV_MAX_F16_ZONES; ++i) {
@@ -734,7 +827,7 @@ __device__ __forceinline__ void own_range(const Params& p, float* smem, int wg) 
     }
     // this wave's share of both kinds (at most 2^22 items in 512 parts: 32 bits)
     const uint32_t parts = p.own_ranges * p.own_waves, part = p.own_waves == 1 ? split : split * kWaves + wave;
-    const int nb = (len + kBlockTokens - 1) / kBlockTokens - s0, np = (nb + 1) >> 1;
+    const int nb = all - s0, np = (nb + 1) >> 1;
     const int x0 = (uint32_t)np * part / parts, x1 = (uint32_t)np * (part + 1) / parts;
     const int f0 = (uint32_t)tiles * part / parts, f1 = (uint32_t)tiles * (part + 1) / parts;
     const int w0 = s0 + 2 * x0, w1 = s0 + min(2 * x1, nb);
@@ -742,12 +835,9 @@ __device__ __forceinline__ void own_range(const Params& p, float* smem, int wg) 
     const int ids = w1 > w0 ? request_ids(row, w0, min(kWindow, w1 - w0)) : 0;
     f4 acc[1][8];
     float m[1] = {0.f}, l[1] = {0.f};
-#pragma unroll
-    for (int n = 0; n < 8; ++n) acc[0][n] = f4{0.f, 0.f, 0.f, 0.f};
     bool fresh = true;
     Range range;
-    attend_int4<1>(p, row, ids, h, w0, w1, len, ln, [&]() { query_to_f16(p, qw); },
-                   [&](int, int j) { return __builtin_bit_cast(h8, qw[j]); }, fresh, range, acc, m, l);
+    own_rows(p, h, row, ids, w0, w1, len, ln, qw, fresh, range, acc, m, l);
     if (f1 > f0) {
         h8 qf[4];
 #pragma unroll
@@ -755,6 +845,13 @@ __device__ __forceinline__ void own_range(const Params& p, float* smem, int wg) 
         attend_f16(p, b, h, lens, f0, f1, ln, qf, fresh, range, acc, m, l);
     }
     float* states = p.states + ((int64_t)(p.prefix_ranges + split) * p.B + b) * Hq * kState + (int64_t)h * p.nrep * kState;
+    int none = 0;        // prefix states that the sequence has no part in
+    bool strays = false;
+    if constexpr (kJoin) {
+        const int count = p.prefix_ranges > 0 ? shared_count(p, b / p.group) : 0;
+        none = count > 0 && len >= count * kBlockTokens ? 0 : p.prefix_ranges;
+        strays = p.strays > 0 && Strays(p, len, count).any();
+    }
     if (p.own_waves == 1) {
         const float sum = row_sum(l[0]);
         if (ln.c < p.nrep) {
@@ -769,14 +866,16 @@ __device__ __forceinline__ void own_range(const Params& p, float* smem, int wg) 
             if (!__builtin_amdgcn_readfirstlane(last)) return;
             for (int r = 0; r < p.nrep; r += 4) {   // two rows at a time and half wave
                 int rows[2], seq[2], firsts[2];
+                bool stray[2];
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const int i = r + 2 * k + (lane >> 5);
                     seq[k] = b;
-                    firsts[k] = s0 > 0 ? 0 : p.prefix_ranges;
+                    firsts[k] = none;
+                    stray[k] = strays;
                     rows[k] = i < p.nrep ? b * Hq + h * p.nrep + i : -1;
                 }
-                join_rows<2>(p, rows, seq, firsts, (lane & 31) * 4);
+                join_rows<2>(p, rows, seq, firsts, stray, (lane & 31) * 4);
             }
         }
     } else {
@@ -791,8 +890,9 @@ __device__ __forceinline__ void own_range(const Params& p, float* smem, int wg) 
             __syncthreads();
             if (!*last) return;
             const int i = threadIdx.x >> 5;
-            const int row[1] = {i < p.nrep ? b * Hq + h * p.nrep + i : -1}, seq[1] = {b}, first[1] = {s0 > 0 ? 0 : p.prefix_ranges};
-            join_rows<1>(p, row, seq, first, (threadIdx.x & 31) * 4);
+            const int row[1] = {i < p.nrep ? b * Hq + h * p.nrep + i : -1}, seq[1] = {b}, first[1] = {none};
+            const bool stray[1] = {strays};
+            join_rows<1>(p, row, seq, first, stray, (threadIdx.x & 31) * 4);
         }
     }
 }
@@ -825,19 +925,18 @@ __global__ __launch_bounds__(kCombine * 64) void shared_combine_kernel(Params p)
     const int64_t stride = (int64_t)p.B * Hq * kState;   // between a row's states
     static_assert(2 * kMaxRanges <= kCombine * 64 && kFewStates <= 64, "a lane for every state");
     const float* st = p.states + (int64_t)row * kState + part * stride;
-    const int k = (p.prefix_ranges + p.own_ranges - part + kWavesRow - 1) / kWavesRow;   // this wave's states
-    float M = -INFINITY, L = 0.f, o0 = 0.f, o1 = 0.f;
-    if (k > 0) {
+    // the sums of states [from, n) of every kWavesRow-th one at `at`; from(): asked for when the states
+    // are on their way
+    const auto sum_states = [&](const float* at, int n, const auto& from, float& M, float& L, float& o0, float& o1) {
+        M = -INFINITY;
+        L = o0 = o1 = 0.f;
+        if (n <= 0) return;
         f2 ml = {-INFINITY, 0.f};
-        if (lane < k) ml = *(const f2*)(st + lane * kWavesRow * stride + kHeadDim);
+        if (lane < n) ml = *(const f2*)(at + lane * kWavesRow * stride + kHeadDim);
         f2 o[8];   // eight states on their way; past the last one it again, with weight 0
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = *(const f2*)(st + min(j, k - 1) * kWavesRow * stride + 2 * lane);
-        // A sequence that does not hold the shared blocks has no part in the prefix's states, which
-        // may hold anything.  (Asked for after the states: their loads do not wait for this.)
-        const int count = p.prefix_ranges > 0 ? shared_count(p, b / p.group) : 0;
-        const bool prefix = count > 0 && row_len(p, b) >= count * kBlockTokens;
-        const int first = prefix ? 0 : (p.prefix_ranges - part + kWavesRow - 1) / kWavesRow;
+        for (int j = 0; j < 8; ++j) o[j] = *(const f2*)(at + min(j, n - 1) * kWavesRow * stride + 2 * lane);
+        const int first = from();
         if (lane < first) ml = f2{-INFINITY, 0.f};
         M = ml.x;
 #pragma unroll
@@ -846,16 +945,34 @@ __global__ __launch_bounds__(kCombine * 64) void shared_combine_kernel(Params p)
         L = ml.y * e;
 #pragma unroll
         for (int x = 1; x < 64; x <<= 1) L += __shfl_xor(L, x);
-        for (int i = 0; i < k; i += 8) {
+        for (int i = 0; i < n; i += 8) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(e), min(i + j, 63)));   // past k: 0
-                const bool in = i + j >= first && i + j < k;   // (past k: state k - 1 may have no part either)
+                const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(e), min(i + j, 63)));   // past n: 0
+                const bool in = i + j >= first && i + j < n;   // (past n: state n - 1 may have no part either)
                 o0 = __builtin_fmaf(in ? o[j].x : 0.f, w, o0);
                 o1 = __builtin_fmaf(in ? o[j].y : 0.f, w, o1);
-                if (i + 8 < k) o[j] = *(const f2*)(st + min(i + 8 + j, k - 1) * kWavesRow * stride + 2 * lane);
+                if (i + 8 < n) o[j] = *(const f2*)(at + min(i + 8 + j, n - 1) * kWavesRow * stride + 2 * lane);
             }
         }
+    };
+    const auto part_of = [&](int n) { return (n - part + kWavesRow - 1) / kWavesRow; };   // this wave's of n states
+    const int T = p.prefix_ranges + p.own_ranges;
+    float M, L, o0, o1;
+    // A sequence that does not hold the shared blocks has no part in the prefix's states, which may
+    // hold anything.
+    sum_states(st, part_of(T), [&]() {
+        const int count = p.prefix_ranges > 0 ? shared_count(p, b / p.group) : 0;
+        return count > 0 && row_len(p, b) >= count * kBlockTokens ? 0 : part_of(p.prefix_ranges);
+    }, M, L, o0, o1);
+    if (__builtin_expect(p.strays > 0 && Strays(p, row_len(p, b), shared_count(p, b / p.group)).any(), 0)) {
+        float M2, L2, p0, p1;
+        sum_states(st + T * stride, part_of(p.strays), []() { return 0; }, M2, L2, p0, p1);
+        const float top = fmaxf(M, M2), w = M == -INFINITY ? 0.f : fast_exp2(M - top), w2 = M2 == -INFINITY ? 0.f : fast_exp2(M2 - top);
+        M = top;
+        L = __builtin_fmaf(L2, w2, L * w);
+        o0 = __builtin_fmaf(p0, w2, o0 * w);
+        o1 = __builtin_fmaf(p1, w2, o1 * w);
     }
     if constexpr (kWavesRow > 1) {
         __shared__ float sm[kWavesRow][kHeadDim + 2];
@@ -901,7 +1018,7 @@ int num_cus() {
 
 struct Plan {
     int tiles, row_tiles;          // row tiles per workgroup, workgroups of rows
-    int prefix_ranges, own_ranges, own_waves;
+    int prefix_ranges, own_ranges, own_waves, strays;
     int64_t prefix_wgs, own_wgs;
     bool own_first;
     double end;                    // of the workgroups, in us, as modelled
@@ -928,7 +1045,7 @@ Plan make_plan(const HkvSharedArgs* s) {
     int64_t items = 0;   // of a sequence's own tokens
     for (int i = 0; i < a->num_f16_zones; ++i) items += ((int64_t)a->f16[i].max_len + kBlockTokens - 1) / kBlockTokens;
     items += ((a->int4_max_len + kBlockTokens - 1) / kBlockTokens - s->shared_blocks + 1) / 2;
-    const bool own = items > 0 || a->int4_lens || s->shared_counts || prefix_pairs == 0;
+    const bool own = items > 0 || prefix_pairs == 0;
     double best = 0;
     for (int o = 1; o <= kMaxRanges; o *= 2) {
         // up to four ranges a wave each, beyond that a workgroup each
@@ -963,6 +1080,8 @@ Plan make_plan(const HkvSharedArgs* s) {
             if (prefix_pairs == 0) break;
         }
     }
+    // (how many there are is not known here: lengths and counts are the device's)
+    p.strays = a->int4_lens || s->shared_counts ? p.prefix_ranges : 0;
     return p;
 }
 
@@ -978,7 +1097,7 @@ bool joins(const HkvSharedArgs* s, const Plan& p) {
 }
 
 size_t state_bytes(const HkvDecodeArgs* a, const Plan& p) {
-    return (size_t)(p.prefix_ranges + p.own_ranges) * a->batch * a->num_q_heads * kState * sizeof(float);
+    return (size_t)(p.prefix_ranges + p.own_ranges + p.strays) * a->batch * a->num_q_heads * kState * sizeof(float);
 }
 
 int check_shared(const HkvSharedArgs* s) {
@@ -1052,6 +1171,7 @@ extern "C" int hkv_shared_attn(const HkvSharedArgs* s, void* stream) {
     p.row_tiles = plan.row_tiles;
     p.prefix_ranges = plan.prefix_ranges;
     p.own_ranges = plan.own_ranges;
+    p.strays = plan.strays;
     p.own_waves = plan.own_waves;
     p.prefix_wgs = (int)plan.prefix_wgs;
     p.own_wgs = (int)plan.own_wgs;
