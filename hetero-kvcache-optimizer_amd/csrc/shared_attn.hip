@@ -1126,6 +1126,12 @@ extern "C" size_t hkv_shared_workspace_bytes(const HkvSharedArgs* s) {
     return state_bytes(&s->decode, make_plan(s));
 }
 
+extern "C" int hkv_shared_launches(const HkvSharedArgs* s) {
+    clear_error();
+    if (check_shared(s) != HKV_OK) return 0;
+    return joins(s, make_plan(s)) ? 1 : 2;
+}
+
 extern "C" int hkv_shared_attn(const HkvSharedArgs* s, void* stream) {
     clear_error();
     int rc = check_shared(s);

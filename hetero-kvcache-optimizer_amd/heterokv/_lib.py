@@ -201,6 +201,7 @@ SYMBOLS = [
     ("hkv_decode_ranges", ctypes.c_int, [ctypes.POINTER(DecodeArgs), ctypes.POINTER(i32)]),
     ("hkv_decode_attn_noalloc", ctypes.c_int, [ctypes.POINTER(DecodeArgs), vp]),
     ("hkv_shared_workspace_bytes", ctypes.c_size_t, [ctypes.POINTER(SharedArgs)]),
+    ("hkv_shared_launches", ctypes.c_int, [ctypes.POINTER(SharedArgs)]),
     ("hkv_shared_attn", ctypes.c_int, [ctypes.POINTER(SharedArgs), vp]),
     ("hkv_prefill_workspace_bytes", ctypes.c_size_t, [i32, i32, i32]),
     ("hkv_prefill_split_bytes", ctypes.c_size_t, [ctypes.POINTER(PrefillArgs)]),

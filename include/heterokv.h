@@ -405,6 +405,8 @@ typedef struct HkvSharedArgs {
 
 /* Reads the sizes of args (and which lengths are given), not its buffers. */
 size_t hkv_shared_workspace_bytes(const HkvSharedArgs* args);
+/* Kernel launches that hkv_shared_attn takes for them: 1 (with arrivals) or 2; 0: bad sizes. */
+int hkv_shared_launches(const HkvSharedArgs* args);
 int hkv_shared_attn(const HkvSharedArgs* args, void* stream);
 
 /*
