@@ -29,6 +29,8 @@ from . import _lib
 from . import ops
 from ._lib import BLOCK_TOKENS, HEAD_DIM, HeteroKVError, check, load, stream_ptr
 
+_WIDE = (torch.uint32, torch.int64, torch.uint64)
+
 
 class BlockTables:
     """Device state: `table` int32 [S, columns] (entries past a row's blocks are -1), `lens`
@@ -105,15 +107,23 @@ class BlockTables:
 
     def _rows(self, x, what, least, most):
         """One int32 per row on the device; host values are checked here, device ones by the kernel."""
+        if isinstance(x, torch.Tensor) and (x.is_floating_point() or x.is_complex()):
+            raise HeteroKVError(-1, "%s: integers expected, one for each of %d rows" % (what, self.num_sequences))
         if isinstance(x, torch.Tensor) and x.device.type != "cpu":
-            if x.numel() != self.num_sequences or x.is_floating_point() or x.is_complex():
-                raise HeteroKVError(-1, "%s: %d integers expected, one for each row" % (what, self.num_sequences))
+            if x.numel() != self.num_sequences:
+                raise HeteroKVError(-1, "%s: %d values for %d rows" % (what, x.numel(), self.num_sequences))
             if x.device != self.device:
                 raise HeteroKVError(-1, "%s: a tensor on %s, the tables are on %s" % (what, x.device, self.device))
-            if x.dtype == torch.int64:   # what 32 bits do not hold stays out of range
-                x = x.clamp(-2 ** 31, 2 ** 31 - 1)
+            if x.dtype in _WIDE:   # what 32 bits do not hold stays out of range
+                if x.dtype == torch.uint64:
+                    x = x.view(torch.int64)
+                    x = torch.where(x < 0, 2 ** 31 - 1, x)
+                x = x.to(torch.int64).clamp(-2 ** 31, 2 ** 31 - 1)
             return x if x.dtype == torch.int32 and x.is_contiguous() else x.reshape(-1).to(torch.int32).contiguous()
-        x = [int(v) for v in (x.reshape(-1).tolist() if isinstance(x, torch.Tensor) else x)]
+        try:
+            x = [operator.index(v) for v in (x.reshape(-1).tolist() if isinstance(x, torch.Tensor) else x)]
+        except TypeError:
+            raise HeteroKVError(-1, "%s: integers expected, one for each of %d rows" % (what, self.num_sequences))
         if len(x) != self.num_sequences or any(v < least or v > most for v in x):
             raise HeteroKVError(-1, "%s: %d values in [%d, %d] expected, one for each row" %
                                 (what, self.num_sequences, least, most))

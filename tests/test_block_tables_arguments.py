@@ -1,0 +1,68 @@
+"""What BlockTables takes for a row's number or token count: whole numbers of any type, host or
+device, and nothing that would have to be cut or wrapped to become one."""
+import types
+
+import pytest
+import torch
+
+DEV = "cuda:0"
+BAD = [[0, 1.5, 2], [0, 0.0, 2], [0, None, 2], [0, "1", 2], [0, 1], [0, 1, 2, 0], [0, 1, 2 ** 32], [0, -2, 1], 1.0, None, "012",
+       [0, 1, 3], [0, [1], 2], torch.tensor([0.9, 1, 2]), torch.tensor([0, 1, 2], dtype=torch.complex64),
+       torch.tensor([0, 1, 2 ** 32 - 1], dtype=torch.uint32), torch.tensor([0, 1, 2 ** 64 - 1], dtype=torch.uint64)]
+GOOD = [[0, 1, 2], (0, 1, 2), range(3), [False, True, 2], torch.arange(3), torch.arange(3, dtype=torch.uint8), torch.arange(3)[:, None],
+        torch.tensor([0, 1, 2], dtype=torch.uint32), torch.tensor([0, 1, 2], dtype=torch.uint64), [torch.tensor(0), 1, 2]]
+
+
+@pytest.mark.parametrize("i", range(len(BAD) + len(GOOD)))
+def test_host_values(i):
+    from heterokv import BlockTables, HeteroKVError
+    rows = types.SimpleNamespace(num_sequences=3, device=torch.device("cpu"))
+    x = (BAD + GOOD)[i]
+    if i >= len(BAD):
+        assert BlockTables._rows(rows, x, "rows", -1, 2).tolist() == [0, 1, 2]
+    else:
+        with pytest.raises(HeteroKVError):
+            BlockTables._rows(rows, x, "rows", -1, 2)
+
+
+def test_host_arrays():
+    numpy = pytest.importorskip("numpy")
+    from heterokv import BlockTables, HeteroKVError
+    rows = types.SimpleNamespace(num_sequences=3, device=torch.device("cpu"))
+    assert BlockTables._rows(rows, numpy.arange(3, dtype=numpy.uint16), "rows", -1, 2).tolist() == [0, 1, 2]
+    with pytest.raises(HeteroKVError):
+        BlockTables._rows(rows, numpy.array([0.0, 1.0, 2.0]), "rows", -1, 2)
+
+
+@pytest.mark.gpu
+def test_calls_and_device_values():
+    import heterokv
+    from heterokv import HeteroKVError, ops
+    t = heterokv.BlockTables(ops.Int4Pool(50, 1, DEV), 3, 200)
+    t.extend([20, 40, 5])
+    before = t.state.clone()
+    for bad in BAD:
+        for call in (t.select, t.extend):
+            if call == t.extend and bad in ([0, 1, 3],):
+                continue     # a good count of tokens
+            with pytest.raises(HeteroKVError):
+                call(bad)
+    for dtype in (torch.uint32, torch.uint64, torch.int64):
+        for x in ([0, 1, 2 ** 32 - 1], [0, 1, 2 ** 31], [0, 1, 2 ** 64 - 1], [0, 1, 2 ** 63], [0, 1, 2 ** 32 + 1]):
+            if max(x) > torch.iinfo(dtype).max:
+                continue
+            for call in (t.select, t.extend):
+                call(torch.tensor(x, dtype=dtype).to(DEV))
+                with pytest.raises(HeteroKVError):
+                    t.check_errors()
+    for bad in (torch.zeros(3, device=DEV), torch.zeros(2, dtype=torch.uint32, device=DEV)):
+        with pytest.raises(HeteroKVError):
+            t.select(bad)
+    torch.cuda.synchronize()
+    assert torch.equal(t.state, before)
+    for dtype in (torch.uint8, torch.int8, torch.int16, torch.uint16, torch.int32, torch.uint32, torch.int64, torch.uint64):
+        t.select(torch.tensor([0, 1, 2], dtype=dtype).to(DEV))
+        wide = torch.tensor([[0, 9], [1, 9], [2, 9]], dtype=dtype).to(DEV)[:, 0]
+        t.select(wide)
+        t.check_errors()
+        assert torch.equal(t.state, before)
