@@ -72,7 +72,8 @@ class BlockTables:
         self.table = table.view(self.num_sequences, self.columns)
         self.err = err if err is not None else ops.ErrorWord(self.device)
         self._records = [q.data for q in self.pools]   # held: their addresses are the kernels'
-        self._pool_ptrs = torch.tensor([q.data.data_ptr() for q in self.pools], dtype=torch.int64).to(self.device)
+        self._addresses = [r.data_ptr() for r in self._records]
+        self._pool_ptrs = torch.tensor(self._addresses, dtype=torch.int64).to(self.device)
         self._lib = load()
         nbytes = self._lib.hkv_blocks_workspace_bytes(self.num_sequences, self.num_blocks)
         self._ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
@@ -98,10 +99,12 @@ class BlockTables:
             self.free[-1:].fill_((1 << (self.num_blocks % 32)) - 1)
 
     def copy_(self, other):
-        """Take the tables, lengths and counts of `other` (of the same sizes), to go back to
+        """Take the tables, lengths and counts of `other` (of the same pools and sizes), to go back to
         them: the records that rows of `other` held have to be as they were."""
         if (other.num_sequences, other.columns, other.num_blocks) != (self.num_sequences, self.columns, self.num_blocks):
             raise HeteroKVError(-1, "BlockTables.copy_: other sizes")
+        if other._addresses != self._addresses:
+            raise HeteroKVError(-1, "BlockTables.copy_: tables of other pools")
         self.state.copy_(other.state)
         return self
 

@@ -66,3 +66,20 @@ def test_calls_and_device_values():
         t.select(wide)
         t.check_errors()
         assert torch.equal(t.state, before)
+
+
+@pytest.mark.gpu
+def test_tables_of_other_pools_are_not_taken_back():
+    import heterokv
+    from heterokv import HeteroKVError, ops
+    pools = [ops.Int4Pool(20, 1, DEV) for _ in range(2)]
+    t = heterokv.BlockTables(pools, 3, 64)
+    t.extend([20, 5, 0])
+    before = t.state.clone()
+    for other in ([ops.Int4Pool(20, 1, DEV) for _ in range(2)], pools[:1], pools[::-1], [pools[0], pools[0]]):
+        with pytest.raises(HeteroKVError, match="pools"):
+            t.copy_(heterokv.BlockTables(other, 3, 64))
+    assert torch.equal(t.state, before)
+    saved = heterokv.BlockTables(pools, 3, 64).copy_(t)
+    t.select([1, 1, 1])
+    assert torch.equal(t.copy_(saved).state, before)
