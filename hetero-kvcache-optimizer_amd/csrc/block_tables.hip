@@ -437,7 +437,8 @@ int check(const HkvBlockTables* t, const char* name, Params& p) {
     p.run = (p.W + kPlan - 1) / kPlan;
     p.L = t->num_pools;
     p.vecs = t->num_kv_heads * (kHeadPartBytes / 16);
-    p.colwgs = (p.stride + kColumns - 1) / kColumns;
+    // a row holds num_blocks blocks at most, its further columns are never in use
+    p.colwgs = ((p.stride < p.N ? p.stride : p.N) + kColumns - 1) / kColumns;
     return HKV_OK;
 }
 

@@ -19,6 +19,7 @@ DTYPE_F16, DTYPE_BF16, DTYPE_F32, DTYPE_U8 = 0, 1, 2, 3
 MAX_F16_ZONES = 3
 MAX_SEQUENCES = 1024   # HKV_MAX_SEQUENCES
 MAX_TABLE_BLOCKS = 1 << 25   # HkvBlockTables.num_blocks
+MAX_TABLE_COLUMNS = 1 << 26   # HkvBlockTables.table_stride
 DECODE_DETERMINISTIC = 1   # HKV_DECODE_DETERMINISTIC
 DECODE_AGENT_HANDOFF = 2   # HKV_DECODE_AGENT_HANDOFF
 DECODE_SCRATCH_BYTES = 8 << 20   # HKV_DECODE_SCRATCH_BYTES (hkv_decode_attn_noalloc)

@@ -59,7 +59,8 @@ class BlockTables:
         self.device = p.device
         self.num_sequences, self.num_blocks = int(num_sequences), p.num_blocks
         self.columns = (int(max_tokens) + BLOCK_TOKENS - 1) // BLOCK_TOKENS
-        if self.num_sequences * self.columns >= 2 ** 31 or p.num_blocks > _lib.MAX_TABLE_BLOCKS:
+        if (self.num_sequences * self.columns >= 2 ** 31 or self.columns > _lib.MAX_TABLE_COLUMNS or
+                p.num_blocks > _lib.MAX_TABLE_BLOCKS):
             raise HeteroKVError(-1, "BlockTables: %d rows of %d blocks out of %d are too many" %
                                 (self.num_sequences, self.columns, p.num_blocks))
         words = (p.num_blocks + 31) // 32

@@ -581,7 +581,8 @@ typedef struct HkvBlockTables {
     uint32_t* free_bits;           /* [ceil(num_blocks / 32)] */
     uint8_t* const* pools;         /* device array: num_pools addresses, 16-byte aligned */
     int64_t num_blocks;            /* records of every pool, <= 2^25 */
-    int32_t num_sequences, table_stride, num_pools, num_kv_heads, head_dim;   /* table below 2^31 entries */
+    int32_t num_sequences, table_stride, num_pools, num_kv_heads, head_dim;   /* table below 2^31 entries,
+                                      table_stride <= 2^26 */
     int32_t* err_flag;             /* device int for HKV_ERR_BIT_* (may be NULL) */
     void* workspace;               /* hkv_blocks_workspace_bytes(), 16-byte aligned; no zero fill needed */
     size_t workspace_bytes;

@@ -83,3 +83,27 @@ def test_tables_of_other_pools_are_not_taken_back():
     saved = heterokv.BlockTables(pools, 3, 64).copy_(t)
     t.select([1, 1, 1])
     assert torch.equal(t.copy_(saved).state, before)
+
+
+@pytest.mark.gpu
+def test_rows_of_very_many_columns():
+    """A row may be as long as 2^26 blocks of table, of which it can hold as many as the pool has:
+    1024 threads for every 16 of its columns would be 2^32, more than a launch can have."""
+    import heterokv
+    from heterokv import HeteroKVError, ops
+    pool = ops.Int4Pool(70, 1, DEV)
+    t = heterokv.BlockTables(pool, 1, 2 ** 30)
+    assert t.extend(16 * 69 + 3).tolist() == [0] and t.table[0, :70].tolist() == list(range(70))
+    t.select([0])
+    t.check_errors()
+    assert t.lens.tolist() == [16 * 69 + 3] and t.refs.tolist() == [1] * 70
+    t.select([-1])
+    t.check_errors()
+    assert t.lens.tolist() == [0] and t.refs.tolist() == [0] * 70 and bool((t.table == -1).all())
+    assert t.free.tolist() == [-1, -1, 63]
+    t.extend(100)
+    t.compact()
+    t.check_errors()
+    assert t.table[0, :8].tolist() == list(range(7)) + [-1]
+    with pytest.raises(HeteroKVError, match="too many"):
+        heterokv.BlockTables(pool, 1, 2 ** 30 + 1)
