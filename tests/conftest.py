@@ -14,7 +14,13 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a ROCm GPU (MI355X) and libheterokv.so")
 
 
+# A side stream's kernels have to overlap those of the main stream there.  Streams take the hardware queues
+# in turn: with other tests' streams in front of it, the two may share one and cannot.
+FIRST = "test_decode_beside_a_concurrent_kernel"
+
+
 def pytest_collection_modifyitems(config, items):
+    items.sort(key=lambda item: getattr(item, "originalname", None) != FIRST)   # (a stable sort)
     try:
         import torch
         has_gpu = torch.cuda.is_available()
