@@ -1048,10 +1048,9 @@ Plan make_plan(const HkvSharedArgs* s) {
     const bool own = items > 0 || prefix_pairs == 0;
     double best = 0;
     for (int o = 1; o <= kMaxRanges; o *= 2) {
-        // up to four ranges a wave each, beyond that a workgroup each
+        // up to four ranges a wave each, beyond that (8, 16, ..) a workgroup of eight waves each
         const int waves = o <= 4 ? 1 : kWaves, own_ranges = o <= 4 ? o : o / kWaves;
         if (o > 1 && (!own || o > items)) break;
-        if (o > 4 && o < kWaves) continue;
         const double own_one = kOwnStart + (double)((items + o - 1) / o) * kOwnItem;
         const int64_t own_wgs = own ? (waves == 1 ? (own_units * own_ranges + kWaves - 1) / kWaves : own_units * own_ranges) : 0;
         for (int n = 1; n <= kMaxRanges; ++n) {
