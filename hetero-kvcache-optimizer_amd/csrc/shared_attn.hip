@@ -705,14 +705,16 @@ __device__ __forceinline__ void own_rows(const Params& p, int h, const int32_t* 
                    [&](int, int j) { return __builtin_bit_cast(h8, qw[j]); }, fresh, range, acc, m, l);
 }
 
-// A range's part of the strays of sequences s0 + i, bit i of `which` (buf: behind the last merge).
+// A range's part of the strays of the sequences whose first rows are r0 + i of a group, bit i of `rows`
+// (buf: behind the last merge).
 template <bool kJoin>
-__device__ __forceinline__ void stray_ranges(const Params& p, float* buf, int split, int h, int s0, int count, uint64_t which) {
+__device__ __forceinline__ void stray_ranges(const Params& p, float* buf, int split, int b0, int h, int r0, int count,
+                                             uint64_t rows) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Lane ln{lane & 15, lane >> 4, 8 * (lane & 3)};
     const int Hq = p.Hkv * p.nrep;
-    for (; which != 0; which &= which - 1) {
-        const int b = s0 + __builtin_ctzll(which), len = row_len(p, b);
+    for (; rows != 0; rows &= rows - 1) {
+        const int b = b0 + (r0 + __builtin_ctzll(rows)) / p.nrep, len = row_len(p, b);
         const Strays st(p, len, count);
         const int nb = st.to - st.from, np = (nb + 1) >> 1, parts = p.prefix_ranges * kWaves, part = split * kWaves + wave;
         const int w0 = st.from + 2 * (np * part / parts), w1 = st.from + min(2 * (np * (part + 1) / parts), nb);
@@ -754,8 +756,6 @@ __device__ __forceinline__ void prefix_range(const Params& p, float* smem, int i
     const int n0 = min(kWindow, w1 - w0);
     int ids = n0 > 0 ? request_ids(row, w0, n0) : 0;
     const int R = p.group * p.nrep, r0 = rt * NT * 16;
-    // lane i: the i-th of the sequences (64 at most) whose first rows are in these tiles
-    const int s0 = b0 + (r0 + p.nrep - 1) / p.nrep, ns = min(b0 + p.group, b0 + (r0 + NT * 16 + p.nrep - 1) / p.nrep) - s0;
     u4 qw[4];
     {   // wave nt of the first NT: row tile nt's queries
         const int r = r0 + wave * 16 + ln.c;
@@ -763,9 +763,12 @@ __device__ __forceinline__ void prefix_range(const Params& p, float* smem, int i
         const int b = b0 + (has ? r / p.nrep : 0), hd = h * p.nrep + (has ? r % p.nrep : 0);
         load_query(p.q + (int64_t)b * p.q_sb + (int64_t)hd * p.q_sh + 32 * ln.g, has, qw);
     }
+    // a sequence's strays are for the workgroup that has its first row: lane i looks at row r0 + i
+    const int seq = (r0 + lane) / p.nrep;
+    const bool first = p.strays > 0 && lane < NT * 16 && r0 + lane < R && seq * p.nrep == r0 + lane;
     int lead = count > 0 ? 0 : -1, len = p.int4_max_len;   // (lead -1: nobody holds the shared blocks)
     if (p.int4_lens) {
-        len = min(p.int4_lens[min(s0 + lane, p.B - 1)], p.int4_max_len);
+        len = min(p.int4_lens[b0 + min(seq, p.group - 1)], p.int4_max_len);
         lead = -1;
         for (int i = 0; i < p.group && lead < 0 && count > 0; i += 64) {
             const uint64_t has = __ballot(i + lane < p.group && p.int4_lens[b0 + min(i + lane, p.group - 1)] >= count * kBlockTokens);
@@ -776,9 +779,9 @@ __device__ __forceinline__ void prefix_range(const Params& p, float* smem, int i
             ids = n0 > 0 ? request_ids(row, w0, n0) : 0;
         }
     }
-    const uint64_t strays = __ballot(p.strays > 0 && lane < ns && Strays(p, len, count).any());
+    const uint64_t strays = __ballot(first && Strays(p, len, count).any());
     if (lead >= 0) prefix_rows<NT, kJoin>(p, smem, split, b0, h, r0, row, ids, w0, w1, count, qw);
-    if (__builtin_expect(strays != 0, 0)) stray_ranges<kJoin>(p, smem + query_bytes(NT) / sizeof(float), split, h, s0, count, strays);
+    if (__builtin_expect(strays != 0, 0)) stray_ranges<kJoin>(p, smem + query_bytes(NT) / sizeof(float), split, b0, h, r0, count, strays);
 }
 // Behind prefix_range of a group's only row tile: the merge of the sequences whose last state
 // this workgroup stored.
@@ -961,11 +964,14 @@ __global__ __launch_bounds__(kCombine * 64) void shared_combine_kernel(Params p)
     float M, L, o0, o1;
     // A sequence that does not hold the shared blocks has no part in the prefix's states, which may
     // hold anything.
-    sum_states(st, part_of(T), [&]() {
-        const int count = p.prefix_ranges > 0 ? shared_count(p, b / p.group) : 0;
-        return count > 0 && row_len(p, b) >= count * kBlockTokens ? 0 : part_of(p.prefix_ranges);
+    bool stray = false;
+    sum_states(st, part_of(T), [&]() {   // (asked in every wave: with several a row, T > kFewStates)
+        if (p.prefix_ranges == 0) return 0;
+        const int len = row_len(p, b), count = shared_count(p, b / p.group);
+        stray = p.strays > 0 && Strays(p, len, count).any();
+        return count > 0 && len >= count * kBlockTokens ? 0 : part_of(p.prefix_ranges);
     }, M, L, o0, o1);
-    if (__builtin_expect(p.strays > 0 && Strays(p, row_len(p, b), shared_count(p, b / p.group)).any(), 0)) {
+    if (__builtin_expect(stray, 0)) {
         float M2, L2, p0, p1;
         sum_states(st + T * stride, part_of(p.strays), []() { return 0; }, M2, L2, p0, p1);
         const float top = fmaxf(M, M2), w = M == -INFINITY ? 0.f : fast_exp2(M - top), w2 = M2 == -INFINITY ? 0.f : fast_exp2(M2 - top);
