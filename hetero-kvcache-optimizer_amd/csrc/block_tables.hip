@@ -6,14 +6,14 @@
 // Thread t counts the bits of its kept run of words, one scan over the threads gives the rank of
 // every run's first free block, and each thread lists its own.
 //
-// Each operator decides in one workgroup (the plan kernel), because what it decides depends on
+// Each operator decides in one workgroup (the plan kernel), as what it decides depends on
 // every row and every bit, and does its bulk work, if any, in a second launch over the GPU.
 // Both are bound by latency (launch, a chain of a few dependent loads, one scan for every sum)
 // until the records that select and compact copy outweigh it.  Measured, plan + bulk kernel:
-//   select   64 rows of 2043 tokens, beam step, 4 pools      4.5 + 5.1 us
-//            one row of 28597 tokens to 16, 28 pools         3.9 + 4.4 us
-//   extend   64 rows by a token 4.3 us; 16 rows by up to 8192 (5000 blocks) 7.6 us
-//   compact  4 rows, 1 pool 4.4 + 2.5 us; 974 records of 8 pools, 275 MB 4.8 + 50 us (5.5 TB/s)
+//   select   64 rows of 2043 tokens, beam step, 4 pools      4.5 + 5.0 us
+//            one row of 28597 tokens to 16, 28 pools         4.0 + 4.4 us
+//   extend   64 rows by a token 4.2 us; 16 rows by up to 8192 (5000 blocks) 7.6 us
+//   compact  4 rows, 1 pool 4.5 + 3.6 us; 974 records of 8 pools, 275 MB 4.8 + 50 us (5.5 TB/s)
 #include "hkv_internal.h"
 
 namespace hkv {

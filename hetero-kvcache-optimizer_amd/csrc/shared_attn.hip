@@ -10,14 +10,15 @@
 // Bound.  A prefix token is 138 bytes and 512 R operations per kv head.  At the copy rate
 // (5.13 TB/s) and the rate of a large matrix product (1216 TFLOP/s) these are equal at R = 64:
 // few rows are bound by HBM, many by the matrix cores and, beside them, by the softmax's VALU
-// work and the nibble decode, whose times mostly add to the products'.
+// work and the nibble decode, whose times mostly add to the products' (a third of the matrix
+// cores' cycles lie beside VALU work).
 //
 // Work.  One launch: workgroups for ranges of the prefix and for the sequences' own tokens, every
 // range leaving its state (o[128], m, l) in the workspace.  A sequence need not hold all of the prefix
 // (its length or its group's count is short of it): its own blocks in there, "strays", are
-// attended by the workgroups of the prefix, all of them, behind what they do for the group.  Few states are merged by whoever
-// stores the last one of a (sequence, kv head) (kJoin), many by a second launch.  A wave
-// streams its own run of block pairs, decodes a pair once into MFMA operands and multiplies it
+// attended by the workgroups of the prefix, all of them, behind what they do for the group.  Few
+// states are merged by whoever stores the last one of a (sequence, kv head) (kJoin), many by a
+// second launch.  A wave streams its own run of block pairs, decodes a pair once into MFMA operands and multiplies it
 // with NT tiles of 16 query rows, NT = 1 .. 4: the decode (~150 of ~400 VALU instructions at NT =
 // 4) is paid once for them (a workgroup of more rows holds no more accumulators: 32 registers a
 // tile); q lies in LDS.  With more than 64 rows several workgroups read a range, next to each
@@ -25,12 +26,13 @@
 //
 // Measured (both launches, us; floor: the larger of bytes and operations at the rates above):
 //   samples x heads        shared tokens     us    floor
-//         2 x 32/8                  1024   11.7      0.4   latency: ids, records, merges
-//        16 x 32/8                 28608     29      9.2   5 to the first products, 2.9 a step of two
-//         8 x 28/4                126912     41       15     waves, 3 to merge eight waves, 4 + launch
-//    6 x 10 x 24/8                  6000     31       16     to merge ranges
-//       256 x 32/8                 16384    121       57   680 TFLOP/s in the prefix, then 24 us of
-//                                                          own tokens, 89 MB
+//         2 x 32/8                  1024   11.4      0.4   latency: ids, records, merges
+//        16 x 32/8                 28608     29      9.2   7 to the first step, 4.4 for it and its loads, 2.6
+//         8 x 28/4                126912     39       15     a further one (two waves a SIMD), 6 to merge
+//                                                          eight waves, the last of them 2 behind; launch
+//    6 x 10 x 24/8                  6000     32       16     + 4 to merge ranges
+//       256 x 32/8                 16384    121       57   105 without own tokens (657 TFLOP/s), then
+//                                                          those, 89 MB
 // Tried and not kept: codes staged through LDS with wide loads; K operands of the next step decoded
 // beside the products of this one (spills); 256 rows a workgroup, all waves sharing tiles that are
 // decoded once into LDS: 8% fewer us in the prefix, all of which its four times as many states cost.
@@ -1091,11 +1093,10 @@ Plan make_plan(const HkvSharedArgs* s) {
 }
 
 // A short call of few rows and states: no second launch.  That saves 2 us of the host's 14, which is
-// what an eager short call takes (2 samples of 1024 tokens 14.3 -> 12.2 us), and nothing on the GPU:
-// stores past the L2, a counter and the reads by one workgroup take what a launch does (11.4 and
-// 11.7 us; the same of 2240 tokens 11.3 and 10.5).  More row tiles lose (11 samples of 3 rows, 720
-// tokens: 15.2 and 17.0), more states too (12 of them: 0.7 us for the code alone, 24 KB that few
-// waves run).
+// what an eager short call takes (2 samples of 1024 tokens 13.9 -> 11.8 us, 4 of 512 14.2 -> 11.7), and nothing
+// on the GPU: stores past the L2, a counter and the reads by one workgroup take what a launch does
+// (11.5 and 11.4 us).  More row tiles lost (11 samples of 3 rows, 720 tokens: 15.2 and 17.0), more states too
+// (12 of them: 0.7 us for the code alone, 24 KB that few waves run).
 constexpr double kJoinEnd = 12.0;
 bool joins(const HkvSharedArgs* s, const Plan& p) {
     return s->arrivals && p.end <= kJoinEnd && p.tiles == 1 && p.row_tiles == 1 && p.prefix_ranges + p.own_ranges <= kJoinFew;
