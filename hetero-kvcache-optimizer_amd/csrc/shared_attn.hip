@@ -151,8 +151,8 @@ __device__ __forceinline__ float row_sum(float v) {
 // Online softmax of NT row tiles.  m is a reference, and the scores relative to it, x = s - m, are at
 // most `lim`.  What limits them is fp16: P = 2^x times a token's V scale goes into the products as
 // fp16, so lim + log2 of the largest V scale (or a little more) is kTopP.  Thus P uses fp16's upper end
-// whatever the size of V, and the likeliest token of V scales within a factor of 4 has 22 bits above the
-// subnormals (with P <= V scale, V of some 2^-8 would have 5).  When a score passes lim, m rises
+// whatever the size of V, and the likeliest token of V scales within a factor of 4 has 21 bits above the
+// subnormals (with 2^x <= 1, V of some 2^-8 would have none).  When a score passes lim, m rises
 // until it is kHeadroom below, and the scores a little larger that follow need no new reference and no
 // pass over the accumulators.  `fresh`: a row may have had no score yet, or only -inf, and its m has to
 // go by the first one whatever it is.  One branch for all tiles: with a branch for each, no product

@@ -403,7 +403,7 @@ typedef struct HkvSharedArgs {
     int32_t* arrivals;             /* [batch x num_kv_heads] device, or NULL */
 } HkvSharedArgs;
 
-/* Reads the sizes of args (and which lengths are given), not its buffers. */
+/* Reads the sizes of args, and whether int4_lens and shared_counts are given, not its buffers. */
 size_t hkv_shared_workspace_bytes(const HkvSharedArgs* args);
 /* Kernel launches that hkv_shared_attn takes for them: 1 (with arrivals) or 2; 0: bad sizes. */
 int hkv_shared_launches(const HkvSharedArgs* args);

@@ -76,3 +76,44 @@ def test_time_of_prefixes_read_alone():
     alone = _us(lambda: c.run(shared_counts=counts))
     print("  %.1f us, one short %.1f us, one group of none %.1f us" % (usual, short, alone), flush=True)
     assert short <= 3 * usual and alone <= 8.5 * usual
+
+
+def test_captured_and_replayed_with_other_lengths():
+    c = Case(62, 2, 6, 32, 8, 960, 40, 16, [30] * 12)
+    lens, counts = c.lens.clone(), torch.tensor([60, 60], dtype=torch.int32, device=DEV)
+    out = torch.empty_like(c.q)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.run(out=out, int4_lens=lens, shared_counts=counts)
+    rng = random.Random(4)
+    for step in range(5):
+        keep, n = _lens(c, rng)
+        lens.copy_(torch.tensor(keep, dtype=torch.int32))
+        counts.copy_(torch.tensor(n, dtype=torch.int32))
+        out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, c.check(keep=keep, int4_lens=lens, shared_counts=counts))
+
+
+def test_two_graphs_of_one_workspace():
+    c, d = Case(63, 1, 16, 32, 8, 3200, 50), Case(64, 2, 3, 28, 4, 640, 60, 16, [20] * 6, dtype=BF16)
+    rng, ws, graphs = random.Random(5), torch.empty(64 << 20, dtype=torch.uint8, device=DEV), []
+    outs = torch.empty_like(c.q), torch.empty_like(d.q)
+    args = [dict(zip(("int4_lens", "shared_counts"), (torch.tensor(x, dtype=torch.int32, device=DEV) for x in _lens(y, rng)))) for y in (c, d)]
+    want = [x.check(keep=a["int4_lens"].tolist(), **a) for x, a in zip((c, d), args)]
+    torch.cuda.synchronize()
+    for x, a, out in zip((c, d), args, outs):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            x.run(out=out, workspace=ws, **a)
+    for step in range(4):
+        ws.fill_(255)
+        for g in graphs if step % 2 else graphs[::-1]:
+            g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+        for out in outs:
+            out.zero_()
